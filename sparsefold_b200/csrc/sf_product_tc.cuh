@@ -801,17 +801,32 @@ __device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, uint32_t*
 __device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// PAIR: the load of one CTA of a pair, whose barrier may be the other one's.
+template <bool PAIR>
 __device__ __forceinline__ void load3(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void load4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
 }
 
 __device__ __forceinline__ uint32_t mma_desc(const Params& p, int rows) {
@@ -885,7 +900,7 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
   }
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      tc::mbar_init(&full[s], CTAS == 2 && rank == 0 ? 2 : 1);   // the even CTA's: its own stage and the other's
+      tc::mbar_init(&full[s], 1);                                // CTAS 2: the even CTA's counts the bytes of both
       tc::mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -913,7 +928,9 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
   // Its instructions count where tiles are small (see issue_half), so how the operands arrive is decided outside the
   // K loop (24 x 4096 -> 2 x 4096: 24.6 us with the choices inside, 20.9 so).
   auto produce = [&](uint32_t from, int every) {
-    const uint32_t fbar = tc::smem_u32(full), ebar = tc::smem_u32(empty);
+    // CTAS 2: both CTAs' loads complete on the even CTA's barrier, which is what orders the odd CTA's bytes before the MMA
+    const uint32_t fbar = CTAS == 2 ? tc::map_shared(full, 0) : tc::smem_u32(full), ebar = tc::smem_u32(empty);
+    const uint32_t own = tc::smem_u32(full);
     const uint32_t stages = (uint32_t)p.stages;
     uint32_t slot = from, parity = 1;
     for (int w = first_item; w < p.items && !aborted; w += step) {
@@ -938,7 +955,7 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
             for (; kb < len; kb += every, k0 += every * BK, ++loads) {
               if (!wait_at(ebar + 8 * slot, parity, p.status, aborted)) return;
               const uint32_t bar = fbar + 8 * slot, sa = sbase + slot * (uint32_t)stage_bytes;
-              expect_at(bar, p.tx);
+              if (CTAS == 1 || rank == 0) expect_at(own + 8 * slot, p.tx * CTAS);
               load_a(sa, bar, k0, pa);
               load_b(sa + p.a_slot, bar, k0, pb);
               if ((slot += every) >= stages) slot -= stages, parity ^= 1;
@@ -947,15 +964,15 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
           }
         }
       };
-      auto a_rows = [&](uint32_t at, uint32_t bar, int k0, int pl) { load3(at, &tmA, bar, k0, m0, pl); };
-      auto a_runs = [&](uint32_t at, uint32_t bar, int k0, int pl) { load4(at, &tmA, bar, 0, k0, m0 / 64, pl); };
+      auto a_rows = [&](uint32_t at, uint32_t bar, int k0, int pl) { load3<CTAS == 2>(at, &tmA, bar, k0, m0, pl); };
+      auto a_runs = [&](uint32_t at, uint32_t bar, int k0, int pl) { load4<CTAS == 2>(at, &tmA, bar, 0, k0, m0 / 64, pl); };
       auto b_rows = [&](uint32_t at, uint32_t bar, int k0, int pl) {
-        load3(at, mapB, bar, k0, n0, pl);
-        if (GATED && CTAS == 1) load3(at + second, &tmB2, bar, k0, n0, pl);
+        load3<CTAS == 2>(at, mapB, bar, k0, n0, pl);
+        if (GATED && CTAS == 1) load3<CTAS == 2>(at + second, &tmB2, bar, k0, n0, pl);
       };
       auto b_runs = [&](uint32_t at, uint32_t bar, int k0, int pl) {
-        load4(at, mapB, bar, 0, k0, n0 / 64, pl);
-        if (GATED && CTAS == 1) load4(at + second, &tmB2, bar, 0, k0, n0 / 64, pl);
+        load4<CTAS == 2>(at, mapB, bar, 0, k0, n0 / 64, pl);
+        if (GATED && CTAS == 1) load4<CTAS == 2>(at + second, &tmB2, bar, 0, k0, n0 / 64, pl);
       };
       if (!p.a_mn && !p.b_mn) stream(a_rows, b_rows);
       else if (!p.a_mn && p.b_one) stream(a_rows, b_runs);
@@ -966,15 +983,15 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
               if (!p.a_mn) a_rows(at, bar, k0, pl);
               else if (p.a_one) a_runs(at, bar, k0, pl);
               else
-                for (int i = 0; i < p.a_boxes; ++i) load3(at + i * 8192, &tmA, bar, m0 + 64 * i, k0, pl);
+                for (int i = 0; i < p.a_boxes; ++i) load3<CTAS == 2>(at + i * 8192, &tmA, bar, m0 + 64 * i, k0, pl);
             },
             [&](uint32_t at, uint32_t bar, int k0, int pl) {
               if (!p.b_mn) b_rows(at, bar, k0, pl);
               else if (p.b_one) b_runs(at, bar, k0, pl);
               else
                 for (int i = 0; i < rows; i += 64) {
-                  load3(at + i * 128, mapB, bar, n0 + i, k0, pl);
-                  if (GATED && CTAS == 1) load3(at + second + i * 128, &tmB2, bar, n0 + i, k0, pl);
+                  load3<CTAS == 2>(at + i * 128, mapB, bar, n0 + i, k0, pl);
+                  if (GATED && CTAS == 1) load3<CTAS == 2>(at + second + i * 128, &tmB2, bar, n0 + i, k0, pl);
                 }
             });
     }
@@ -990,15 +1007,7 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
   } else if (warp == EPI_WARPS + 1 && lane == 0) {
     uint32_t it = 0;
     Ring r;
-    if (CTAS == 2 && rank == 1) {
-      // ---- the odd CTA passes on which of its stages have landed ----
-      for (int w = first_item; w < p.items && !aborted; w += step) {
-        for (int i = split_blocks(p, w % p.splits) * p.pairs; i > 0; --i, r.next(p.stages)) {
-          if (!tc::mbar_wait(&full[r.slot], r.phase, p.status, aborted)) break;
-          tc::mbar_arrive_cluster(tc::map_shared(&full[r.slot], 0));
-        }
-      }
-    } else {
+    if (CTAS == 1 || rank == 0) {
       // ---- MMA issuer (stops at its first failed wait) ----
       const uint32_t idesc = mma_desc(p, BM * CTAS);
       const uint64_t a_desc = first_desc(sbase, p.a_mn), b_desc = first_desc(sbase + p.a_slot, p.b_mn);
@@ -1017,7 +1026,9 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
           const int steps = min(p.seg_kb, blocks - seg) * p.pairs;
           for (int i = 0; i < steps; ++i, r.next(p.stages)) {
             const uint32_t s = r.slot;
-            if (!tc::mbar_wait(&full[s], r.phase, p.status, aborted)) break;
+            if (!(CTAS == 2 ? tc::mbar_wait_pair(&full[s], r.phase, p.status, aborted)
+                            : tc::mbar_wait(&full[s], r.phase, p.status, aborted)))
+              break;
             tc::tc_fence_after();
             // K-major: 16 elements = 32 bytes along the swizzled rows; M/N-major: 16 rows of 128 bytes
             const uint32_t at = (s * (uint32_t)stage_bytes) >> 4;
@@ -1103,7 +1114,8 @@ __global__ void __launch_bounds__(threads_of(STAGED), 1) k_product_tc(const __gr
         for (uint32_t j = loads > half ? loads - half : 0u; j < loads; ++j)
           tc::mbar_wait_drain(&full[(part + 2 * j) % p.stages], (part + 2 * j) / p.stages & 1, p.status);
     } else if (warp == EPI_WARPS && lane == 0) {
-      tc::drain_ring(full, p.stages, loads, p.status);
+      // the odd CTA's loads complete on the even one's barriers: it waits until the MMAs have read them
+      tc::drain_ring(CTAS == 2 && rank ? empty : full, p.stages, loads, p.status);
     }
     if (warp == EPI_WARPS + 1 && lane == 0 && rank == 0) {
       if constexpr (CTAS == 2) {

@@ -126,12 +126,11 @@ __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.
 
 // ---- clusters of two (tcgen05 cta_group::2) ------------------------------------------
 // A pair of CTAs shares each MMA: the even one issues it, both hold half of A and B in their
-// shared memory and half of the rows of D in their TMEM.  Loads stay local to each CTA.  What a
-// remote arrival announces is never data in the caches: either a stage of the arriving CTA's own
-// shared memory, which its loads have filled (it has waited for them) and only the tensor cores
-// read, or TMEM columns that its tcgen05.ld have left, ordered by the tcgen05 fences on both
-// sides.  So the arrivals and waits are relaxed: release.cluster and acquire.cluster here cost a
-// fence of all the thread's memory for each stage (16384 x 4096 x 4096: 741 us with them).
+// shared memory and half of the rows of D in their TMEM.  Each CTA loads its own half; both CTAs'
+// loads complete on the even CTA's barrier (the .cta_group::2 form of the load), so the phase that
+// the issuer waits for covers the bytes in both shared memories.  What the odd CTA's threads
+// announce with an arrival of their own is only that their tcgen05.ld have left TMEM columns:
+// tcgen05 operations, ordered by the tcgen05 fences on both sides of a relaxed arrival and wait.
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -156,6 +155,26 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(0u)
+        : "memory");
+    if (ok) return true;
+  }
+  aborted = true;
+  if (status) atomicCAS(status, 0u, (uint32_t)SF_ERR_TIMEOUT);
+  return false;
+}
+// The wait for a stage of both CTAs: acquire at the scope of the cluster, as the bytes are in two CTAs' shared memory
+// (it costs nothing: 8192 x 2048 -> 2 x 8192, forward and gradients, 1498 us a pass; 1570 with a thread of the odd CTA
+// that waited for its stages and reported each).
+__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, uint32_t* status, bool& aborted) {
+  const uint32_t limit = aborted ? 1u : kWaitLimit;
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity), "r"(0u)

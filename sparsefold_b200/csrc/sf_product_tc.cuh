@@ -213,18 +213,20 @@ __device__ __forceinline__ pair_t rcp2(pair_t v) {
 __device__ __forceinline__ pair_t sigmoid2(pair_t z) {
   return rcp2(add2(ex2_2(mul2(z, pk1(-1.4426950408889634f))), pk1(1.0f)));
 }
-// Phi(z) and exp(-z^2 / 2) by Abramowitz & Stegun 7.1.26 (absolute error of erf below 1.5e-7): with x = |z| / sqrt 2
-// and q = erfc(x) / 2, Phi = 1/2 + sign(z) (1/2 - q).
+// Phi(z) and exp(-z^2 / 2) as normal_cdf<true>: q is chosen by the sign of z, not formed as 1 - (1 - q), which would
+// lose it in the negative tail (4 % of gelu at z = -5, all of it at -6).
 __device__ __forceinline__ void cdf2(pair_t z, pair_t& cdf, pair_t& e) {
-  const pair_t x = mul2(z & 0x7FFFFFFF7FFFFFFFull, pk1(0.70710678118654752f));
-  e = ex2_2(mul2(mul2(x, x), pk1(-1.4426950408889634f)));
-  const pair_t t = rcp2(fma2(pk1(0.3275911f), x, pk1(1.0f)));
-  pair_t y = fma2(t, pk1(1.061405429f), pk1(-1.453152027f));
-  y = fma2(t, y, pk1(1.421413741f));
-  y = fma2(t, y, pk1(-0.284496736f));
-  y = fma2(t, y, pk1(0.254829592f));
-  const pair_t h = fma2(mul2(mul2(t, y), e), pk1(-0.5f), pk1(0.5f));      // 1/2 - q, not negative
-  cdf = add2(pk1(0.5f), h ^ (z & 0x8000000080000000ull));
+  e = ex2_2(mul2(mul2(z, z), pk1(-0.72134752044448170f)));
+  const pair_t t = rcp2(fma2(pk1(kTailC), z & 0x7FFFFFFF7FFFFFFFull, pk1(1.0f)));
+  pair_t y = pk1(tail(7));
+#pragma unroll
+  for (int i = 6; i >= 0; --i) y = fma2(t, y, pk1(tail(i)));
+  const pair_t q = mul2(mul2(t, y), e), r = fma2(q, pk1(-1.0f), pk1(1.0f));
+  float z0, z1, q0, q1, r0, r1;
+  unpk(z, z0, z1);
+  unpk(q, q0, q1);
+  unpk(r, r0, r1);
+  cdf = pk(z0 < 0.f ? q0 : r0, z1 < 0.f ? q1 : r1);
 }
 // act(z), and with GRAD act'(z).
 template <int ACT, bool GRAD>

@@ -45,3 +45,32 @@ def test_pairs_of_ctas_give_the_same_bits_every_time(rows, k, n, kn):
     got = ops.linear_act(x, w), *ops.linear_act_backward(dy, x, w)[:2]
     for a, b in zip(got, want):
       assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,k,n", [(4, 16, 48), (20, 16, 48), (20, 4096, 4104), (200, 72, 72), (200, 1200, 77), (9400, 72, 600)])
+def test_gelu_keeps_its_tail(rows, k, n, dtype):
+  """gelu and its derivative between -12 and 6, relatively, on every path (dot products, tiles with and without a staged
+  epilogue, clusters of two, saved pre-activations): z is the bias alone, one value to a column, and dy is one in a
+  single row, so that dbias is the derivative before any rounding to bf16.
+  bf16: one rounding (2^-8) of a value off by 2^-17 of itself; the derivative Phi + z phi by 2^-16 of its two terms.
+  fp32: Phi = erfc / 2, whose argument's rounding 2^-24 x costs 2 x^2 2^-24 of it (x^2 <= 72: 2^-16.8)."""
+  z = torch.cat((torch.linspace(-12, -2, n - 8, device="cuda"), torch.linspace(-1, 6, 8, device="cuda")))
+  x = rnd(1, rows, k).to(dtype)
+  w = torch.zeros(n, k, dtype=dtype, device="cuda")
+  dy = torch.zeros(rows, n, dtype=dtype, device="cuda")
+  dy[rows // 2] = 1.0
+  zd = z.double()
+  phi, cdf = (-0.5 * zd * zd).exp() / (2 * torch.pi) ** 0.5, 0.5 * torch.special.erfc(-zd * 0.5 ** 0.5)
+  a, da = zd * cdf, cdf + zd * phi
+  y, saved = ops.linear_act(x, w, z, activation="gelu", save=True)
+  tol = (2.0 ** -8 if dtype == BF else 0.0) + 2.0 ** -16
+  assert bool(((y.double() - a).abs() <= tol * a.abs()).all())
+  two, one = torch.cat((z, torch.ones_like(z))), torch.cat((w, w))
+  assert bool(((ops.gated_linear(x, one, two, activation="gelu").double() - a).abs() <= tol * a.abs()).all())
+  for s in {id(saved): saved, 0: None}.values():
+    db = ops.linear_act_backward(dy, x, w, z, activation="gelu", saved=s)[2].double()
+    assert bool(((db - da).abs() <= 2.0 ** -16 * (cdf + zd.abs() * phi)).all())
+    db = ops.gated_linear_backward(dy, x, one, two, activation="gelu", saved=None)[2].double()
+    assert bool(((db[:n] - da).abs() <= 2.0 ** -16 * (cdf + zd.abs() * phi)).all())
+    assert bool(((db[n:] - a).abs() <= 2.0 ** -16 * a.abs()).all())

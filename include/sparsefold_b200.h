@@ -349,8 +349,9 @@ size_t sf_layernorm_backward_workspace(int64_t rows, int64_t cols);
  * values do not overflow or underflow on the way), 0: the largest magnitude (a NaN anywhere gives NaN).
  * The sums are formed in a fixed order: the same tensors give the same bits.
  * sf_clip_grad_norm then writes outs[i] = ptrs[i] * min(1, max_norm / (norm + 1e-6)), of ptrs' dtype;
- * outs[i] may equal ptrs[i] (a scale of 1 then writes nothing), but overlap no other tensor.  A NaN norm
- * makes every output NaN, an infinite one zero (NaN where the gradient itself is infinite).
+ * outs[i] may equal ptrs[i] (a scale of 1 then writes nothing), but overlap no other tensor.  The scale is formed in
+ * fp64 and rounded once, so finite gradients whose norm overflows fp32 (*norm is then infinite) are scaled too.  A NaN
+ * makes every output NaN, an infinite gradient makes them zero (itself NaN; with an infinite max_norm all are NaN).
  * ws of sf_grad_norm_workspace() bytes, 256-byte aligned.                                            */
 int sf_grad_norm(const void* const* ptrs, const int64_t* numels, const int32_t* dtypes, int64_t count,
                  int norm_type, float* norm, void* ws, size_t ws_bytes, sf_stream_t stream);

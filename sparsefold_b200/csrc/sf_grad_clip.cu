@@ -207,11 +207,11 @@ __global__ void __launch_bounds__(kThreads, 6) k_grad_norm(const __grid_constant
   }
 }
 
-// The norm from the partials, for every thread of a block: each block adds them in the same order.
-__device__ __forceinline__ float norm_of(const double* __restrict__ part, int parts, int type) {
+// The norm from the partials before its rounding, for every thread of a block: each block adds them in the same order.
+__device__ __forceinline__ double norm_of(const double* __restrict__ part, int parts, int type) {
   __shared__ double s_sum[kThreads / 32];
   __shared__ uint32_t s_most[kThreads / 32];
-  __shared__ float s_norm;
+  __shared__ double s_norm;
   double sum = 0.0;
   uint32_t most = 0;
   for (int i = threadIdx.x; i < parts; i += kThreads) {
@@ -233,7 +233,7 @@ __device__ __forceinline__ float norm_of(const double* __restrict__ part, int pa
       sum += s_sum[w];
       most = max(most, s_most[w]);
     }
-    s_norm = type == 2 ? (float)sqrt(sum) : __uint_as_float(most);
+    s_norm = type == 2 ? sqrt(sum) : (double)__uint_as_float(most);
   }
   __syncthreads();
   return s_norm;
@@ -243,20 +243,21 @@ __global__ void __launch_bounds__(kThreads) k_norm_final(const double* __restric
                                                          float* __restrict__ norm) {
   tc::griddep_wait();
   tc::griddep_launch();
-  const float v = norm_of(part, parts, type);
-  if (threadIdx.x == 0) *norm = v;
+  const double v = norm_of(part, parts, type);
+  if (threadIdx.x == 0) *norm = (float)v;
 }
 
 // Every block forms the norm from the partials itself (a few hundred values from L2), which saves a launch between
-// the two passes.  A block goes through its run from the end: what the first pass read last may still be in L2.
+// the two passes.  The scale comes from the norm in fp64 and is rounded once: its error is in every gradient (from the
+// norm rounded to fp32 and in fp32 it was twice as large, 5.9e-8 of the gradients against 2.9e-8).  A block goes through its run from the end: what the first pass read last may still be in L2.
 template <int N>
 __global__ void __launch_bounds__(kThreads, 8) k_clip(const __grid_constant__ Table<N> t, const double* __restrict__ part,
                                                    int parts, int type, float* __restrict__ norm, float max_norm) {
   tc::griddep_wait();
   tc::griddep_launch();
-  const float nv = norm_of(part, parts, type), q = max_norm / (nv + 1e-6f);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nv;
-  const float scale = q < 1.0f || q != q ? q : 1.0f;
+  const double nv = norm_of(part, parts, type), q = (double)max_norm / (nv + 1e-6);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nv;
+  const float scale = q < 1.0 || q != q ? (float)q : 1.0f;
   const int granules = t.end[t.count - 1], first = run_start(granules, blockIdx.x);
   int g = run_start(granules, blockIdx.x + 1), i = tensor_of(t, g - 1);
   for (; g > first; --i) {

@@ -16,14 +16,18 @@ def _match(g, dtype):
   return None if g is None else g.to(dtype)
 
 
+def _differentiated(*tensors) -> bool:
+  """Whether autograd will ask for a gradient of one of them.  (``ctx.needs_input_grad`` does not say so: it is true for
+  parameters under ``torch.no_grad`` too.)"""
+  return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _LinearAct(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, wt, bias, activation, gated):
-    save = any(ctx.needs_input_grad)
     fn = ops.gated_linear if gated else ops.linear_act
     b32 = None if bias is None else bias.float()
-    got = fn(x, wt, b32, activation=activation, save=save)
-    y, saved = got if save else (got, None)
+    y, saved = fn(x, wt, b32, activation=activation, save=True)
     ctx.save_for_backward(x, wt, bias, saved)
     ctx.form = (activation, gated)
     return y
@@ -64,7 +68,7 @@ class _LayerNorm(torch.autograd.Function):
 def linear_act(x, wt, bias=None, *, activation=None, residual=None):
   """Differentiable ``ops.linear_act``.  Without a gradient to compute, and where the residual is not
   differentiated, the residual is added in the kernel's epilogue; its gradient is dy otherwise too."""
-  if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, wt, bias, residual)):
+  if not _differentiated(x, wt, bias, residual):
     b32 = None if bias is None else bias.float()
     return ops.linear_act(x, wt, b32, activation=activation, residual=residual)
   if residual is None:
@@ -77,26 +81,30 @@ class _LinearActResidual(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, wt, bias, residual, activation):
     b32 = None if bias is None else bias.float()
+    ctx.activation = activation
+    if not any(ctx.needs_input_grad[:3]):     # the residual's gradient is dy and needs nothing kept
+      return ops.linear_act(x, wt, b32, activation=activation, residual=residual)
     y, saved = ops.linear_act(x, wt, b32, activation=activation, residual=residual, save=True)
     ctx.save_for_backward(x, wt, bias, saved)
-    ctx.activation = activation
     return y
 
   @staticmethod
   @once_differentiable
   def backward(ctx, dy):
-    x, wt, bias, saved = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx = dwt = db = None
-    if any(need[:3]):
-      b32 = None if bias is None else bias.float()
-      dx, dwt, db = ops.linear_act_backward(dy, x, wt, b32, activation=ctx.activation, saved=saved, need_dx=need[0],
-                                            need_dwt=need[1], need_dbias=need[2])
+    if not any(need[:3]):
+      return None, None, None, dy, None
+    x, wt, bias, saved = ctx.saved_tensors
+    b32 = None if bias is None else bias.float()
+    dx, dwt, db = ops.linear_act_backward(dy, x, wt, b32, activation=ctx.activation, saved=saved, need_dx=need[0],
+                                          need_dwt=need[1], need_dbias=need[2])
     return dx, dwt, _match(db, bias.dtype if bias is not None else None), dy if need[3] else None, None
 
 
 def gated_linear(x, wt, bias=None, *, activation="silu"):
   """Differentiable ``ops.gated_linear``."""
+  if not _differentiated(x, wt, bias):
+    return ops.gated_linear(x, wt, None if bias is None else bias.float(), activation=activation)
   return _LinearAct.apply(x, wt, bias, activation, True)
 
 

@@ -1,0 +1,53 @@
+"""The differentiable forms and the trainable modules on a machine without a GPU: what they ask of ``ops``, with the
+calls themselves replaced by their formulas."""
+import pytest
+import torch
+
+from sparsefold_b200 import training
+
+ACT = {None: lambda z: z, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}
+
+
+@pytest.fixture
+def calls(monkeypatch):
+  """ops.linear_act and ops.gated_linear as formulas; the list of (name, save) that were called."""
+  seen = []
+
+  def linear_act(x, wt, bias=None, *, activation=None, residual=None, save=False):
+    seen.append(("linear_act", save))
+    y = ACT[activation](torch.nn.functional.linear(x, wt, bias)) + (0 if residual is None else residual)
+    return (y, y.new_zeros(1)) if save else y
+
+  def gated_linear(x, wt, bias=None, *, activation="silu", save=False):
+    seen.append(("gated_linear", save))
+    gate, up = torch.nn.functional.linear(x, wt, bias).chunk(2, -1)
+    return (ACT[activation](gate) * up, gate.new_zeros(1)) if save else ACT[activation](gate) * up
+
+  monkeypatch.setattr(training.ops, "linear_act", linear_act)
+  monkeypatch.setattr(training.ops, "gated_linear", gated_linear)
+  return seen
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_nothing_is_kept_without_a_gradient_to_compute(calls, bias):
+  x, w = torch.randn(3, 8), torch.randn(12, 8, requires_grad=True)
+  b = torch.randn(12, requires_grad=True) if bias else None
+  with torch.no_grad():
+    training.gated_linear(x, w, b)
+    training.linear_act(x, w, b, activation="gelu")
+    training.linear_act(x, w, b, activation="gelu", residual=torch.zeros(3, 12, requires_grad=True))
+  training.gated_linear(x, w.detach(), None if b is None else b.detach())
+  training.linear_act(x, w.detach())
+  assert [save for _, save in calls] == [False] * 5
+  assert training.gated_linear(x, w, b).requires_grad and calls[-1] == ("gated_linear", True)
+
+
+def test_only_the_residual_is_differentiated(calls):
+  x, w, r = torch.randn(3, 8), torch.randn(12, 8), torch.randn(1, 12, requires_grad=True)
+  y = training.linear_act(x, w, activation="silu", residual=r)
+  assert calls == [("linear_act", False)]
+  dy = torch.randn(3, 12)
+  y.backward(dy)
+  assert torch.allclose(r.grad, dy.sum(0, keepdim=True))
+  training.linear_act(x.requires_grad_(True), w, activation="silu", residual=r)
+  assert calls[-1] == ("linear_act", True)

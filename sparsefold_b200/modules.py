@@ -916,12 +916,15 @@ def trainable(module: torch.nn.Module, on: bool = True) -> list[torch.nn.Paramet
   ``training.transition`` on their parameters themselves (not on the packed copies), which get
   requires_grad, and pass gradients to their input.  Returns those parameters.  The other modules stay
   forward-only: their outputs carry no gradient, so in a stack a transition's parameters get one only from
-  what lies between it and the next of those.  ``on=False`` goes back to the fused forward kernel; call
-  ``prepare`` then, so that it sees the trained weights."""
+  what lies between it and the next of those.  ``on=False`` goes back to the fused forward kernel and packs
+  the parameters as they are then for it."""
   params = []
   for m in module.modules():
     if isinstance(m, TransitionBlockB200):
+      trained = getattr(m, "_sf_trainable", False)
       m._sf_trainable = on
+      if trained and not on and getattr(m, "_native_prepared", False):   # its packed copies are from before training
+        m.prepare_native()
       for p in (m.input_layer_norm.weight, m.input_layer_norm.bias, m.transition1.weight, m.transition2.weight):
         p.requires_grad_(on)
         params.append(p)

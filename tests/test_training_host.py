@@ -3,7 +3,7 @@ calls themselves replaced by their formulas."""
 import pytest
 import torch
 
-from sparsefold_b200 import training
+from sparsefold_b200 import modules, synth, training
 
 ACT = {None: lambda z: z, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}
 
@@ -51,3 +51,22 @@ def test_only_the_residual_is_differentiated(calls):
   assert torch.allclose(r.grad, dy.sum(0, keepdim=True))
   training.linear_act(x.requires_grad_(True), w, activation="silu", residual=r)
   assert calls[-1] == ("linear_act", True)
+
+
+def test_the_fused_kernel_sees_the_trained_weights():
+  blk = modules.TransitionBlock(16, 2)
+  synth.init_params(blk, seed=1)
+  modules.trainable(blk)
+  modules.trainable(blk, False)                      # not prepared: nothing to pack, and a call still says so
+  with pytest.raises(RuntimeError, match="prepare"):
+    blk(torch.zeros(2, 16))
+  modules.prepare(blk)
+  params = modules.trainable(blk)
+  with torch.no_grad():
+    for p in params:
+      p.mul_(-2.0)
+  modules.trainable(blk, False)
+  assert torch.equal(blk._packed("w1", torch.float32), blk.transition1.weight.detach().t())
+  assert torch.equal(blk._packed("w2", torch.bfloat16), blk.transition2.weight.detach().t().to(torch.bfloat16))
+  assert torch.equal(blk._kept("ln_w"), blk.input_layer_norm.weight.detach())
+  assert torch.equal(blk._kept("ln_b"), blk.input_layer_norm.bias.detach())

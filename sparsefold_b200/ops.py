@@ -52,8 +52,9 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5) -> torch.Tensor
   x = x.contiguous()
   y = torch.empty_like(x)
   cols = x.shape[-1]
-  N.call("sf_layernorm", _dt(x), _p(x), _p(y), _p(weight), _p(bias), x.numel() // cols, cols,
-         C.c_float(eps), _stream())
+  with _on(x.get_device()):
+    N.call("sf_layernorm", _dt(x), _p(x), _p(y), _p(weight), _p(bias), x.numel() // cols, cols,
+           C.c_float(eps), _stream())
   return y
 
 

@@ -3,7 +3,7 @@ calls themselves replaced by their formulas."""
 import pytest
 import torch
 
-from sparsefold_b200 import modules, synth, training
+from sparsefold_b200 import modules, ops, synth, training
 
 ACT = {None: lambda z: z, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}
 
@@ -70,3 +70,34 @@ def test_the_fused_kernel_sees_the_trained_weights():
   assert torch.equal(blk._packed("w2", torch.bfloat16), blk.transition2.weight.detach().t().to(torch.bfloat16))
   assert torch.equal(blk._kept("ln_w"), blk.input_layer_norm.weight.detach())
   assert torch.equal(blk._kept("ln_b"), blk.input_layer_norm.bias.detach())
+
+
+def test_layer_norm_runs_on_its_tensors_device(monkeypatch):
+  """The launch and its stream belong to x's device, whichever device is current."""
+  current, launched = [0], []
+
+  class Device:
+    def __init__(self, index):
+      self.index = index
+
+    def __enter__(self):
+      self.before, current[0] = current[0], self.index
+
+    def __exit__(self, *_):
+      current[0] = self.before
+
+  class OnOne(torch.Tensor):
+    is_cuda = True
+
+    def get_device(self):
+      return 1
+
+    def contiguous(self):
+      return self
+
+  monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+  monkeypatch.setattr(torch.cuda, "device", Device)
+  monkeypatch.setattr(ops, "_stream", lambda: 100 + current[0])
+  monkeypatch.setattr(ops.N, "call", lambda name, *args: launched.append((name, current[0], args[-1])))
+  ops.layer_norm(torch.zeros(2, 8).as_subclass(OnOne), None, None)
+  assert launched == [("sf_layernorm", 1, 101)] and current == [0]

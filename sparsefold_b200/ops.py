@@ -49,9 +49,14 @@ def mask_u8(mask: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5) -> torch.Tensor:
   _cuda(x, weight, bias)
+  cols = x.shape[-1]
+  for t in (weight, bias):   # the kernel reads [cols] fp32 of each
+    if t is not None and (t.dtype != torch.float32 or t.shape != (cols,) or t.get_device() != x.get_device()):
+      raise ValueError(f"layer_norm: weight and bias must be fp32 [{cols}] on {x.device}, got {t.dtype} "
+                       f"{tuple(t.shape)} on {t.device}")
+  weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
   x = x.contiguous()
   y = torch.empty_like(x)
-  cols = x.shape[-1]
   with _on(x.get_device()):
     N.call("sf_layernorm", _dt(x), _p(x), _p(y), _p(weight), _p(bias), x.numel() // cols, cols,
            C.c_float(eps), _stream())

@@ -72,6 +72,17 @@ def test_the_fused_kernel_sees_the_trained_weights():
   assert torch.equal(blk._kept("ln_b"), blk.input_layer_norm.bias.detach())
 
 
+class OnOne(torch.Tensor):
+  """A host tensor that says it is on the second GPU."""
+  is_cuda = True
+
+  def get_device(self):
+    return 1
+
+  def contiguous(self):
+    return self
+
+
 def test_layer_norm_runs_on_its_tensors_device(monkeypatch):
   """The launch and its stream belong to x's device, whichever device is current."""
   current, launched = [0], []
@@ -86,18 +97,27 @@ def test_layer_norm_runs_on_its_tensors_device(monkeypatch):
     def __exit__(self, *_):
       current[0] = self.before
 
-  class OnOne(torch.Tensor):
-    is_cuda = True
-
-    def get_device(self):
-      return 1
-
-    def contiguous(self):
-      return self
-
   monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
   monkeypatch.setattr(torch.cuda, "device", Device)
   monkeypatch.setattr(ops, "_stream", lambda: 100 + current[0])
   monkeypatch.setattr(ops.N, "call", lambda name, *args: launched.append((name, current[0], args[-1])))
   ops.layer_norm(torch.zeros(2, 8).as_subclass(OnOne), None, None)
   assert launched == [("sf_layernorm", 1, 101)] and current == [0]
+
+
+@pytest.mark.parametrize("bad", [torch.ones(7), torch.ones(9), torch.ones(1, 8), torch.ones(8, dtype=torch.bfloat16),
+                                 torch.ones(8, dtype=torch.float64)], ids=str)
+def test_layer_norm_refuses_other_weights(monkeypatch, bad):
+  """The kernel reads [cols] fp32 values of weight and bias: a shorter one would be read out of range."""
+  monkeypatch.setattr(ops.N, "call", lambda *_: pytest.fail("launched"))
+  x, bad = torch.zeros(2, 8).as_subclass(OnOne), bad.as_subclass(OnOne)
+  for args in ((bad, None), (None, bad)):
+    with pytest.raises(ValueError, match="layer_norm"):
+      ops.layer_norm(x, *args)
+
+  class OnZero(OnOne):
+    def get_device(self):
+      return 0
+
+  with pytest.raises(ValueError, match="layer_norm"):
+    ops.layer_norm(x, torch.ones(8).as_subclass(OnZero), None)

@@ -57,6 +57,8 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5) -> torch.Tensor
   weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
   x = x.contiguous()
   y = torch.empty_like(x)
+  if x.numel() == 0:         # no rows: nothing to launch, and torch gives no address
+    return y
   with _on(x.get_device()):
     N.call("sf_layernorm", _dt(x), _p(x), _p(y), _p(weight), _p(bias), x.numel() // cols, cols,
            C.c_float(eps), _stream())

@@ -3,7 +3,7 @@ repeated calls, forms that the C ABI allows, values at the ends of the activatio
 import pytest
 import torch
 
-from sparsefold_b200 import _native, ops
+from sparsefold_b200 import _native, ops, training
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -74,3 +74,17 @@ def test_gelu_keeps_its_tail(rows, k, n, dtype):
     db = ops.gated_linear_backward(dy, x, one, two, activation="gelu", saved=None)[2].double()
     assert bool(((db[:n] - da).abs() <= 2.0 ** -16 * (cdf + zd.abs() * phi)).all())
     assert bool(((db[n:] - a).abs() <= 2.0 ** -16 * a.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_transition_of_no_rows(dtype):
+  """Outputs and input gradients without rows, zero gradients of the parameters."""
+  x = torch.zeros(2, 0, 24, dtype=dtype, device="cuda", requires_grad=True)
+  lw, lb = (torch.ones(24, device="cuda", requires_grad=True) for _ in range(2))
+  w1, w2 = rnd(1, 64, 24).to(dtype).requires_grad_(True), rnd(2, 24, 32).to(dtype).requires_grad_(True)
+  y = training.transition(x, lw, lb, w1, w2)
+  assert y.shape == x.shape
+  y.sum().backward()
+  assert x.grad.shape == x.shape
+  for p in (lw, lb, w1, w2):
+    assert p.grad.shape == p.shape and not p.grad.any()

@@ -121,3 +121,10 @@ def test_layer_norm_refuses_other_weights(monkeypatch, bad):
 
   with pytest.raises(ValueError, match="layer_norm"):
     ops.layer_norm(x, torch.ones(8).as_subclass(OnZero), None)
+
+
+def test_layer_norm_of_no_rows(monkeypatch):
+  monkeypatch.setattr(ops.N, "call", lambda *_: pytest.fail("launched"))
+  w = torch.ones(8).as_subclass(OnOne)
+  for shape in ((0, 8), (3, 0, 8)):
+    assert ops.layer_norm(torch.zeros(shape).as_subclass(OnOne), w, w).shape == shape

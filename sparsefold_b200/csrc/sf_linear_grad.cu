@@ -159,10 +159,11 @@ __device__ __forceinline__ void dz_rows(const Epi& e, int64_t from, int64_t end,
 }
 
 template <int KIND, int OUT, int V>
-__global__ void __launch_bounds__(128) k_dz(Epi e, int64_t rows) {
+__global__ void __launch_bounds__(128) k_dz(Epi e, int64_t rows, unsigned row_blocks) {
   tc::griddep_wait();
   tc::griddep_launch();
-  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V, blk = blockIdx.x;
+  const unsigned cb = blockIdx.x / row_blocks;      // the blocks of one column range are neighbours
+  const int64_t c = ((int64_t)cb * blockDim.x + threadIdx.x) * V, blk = blockIdx.x - cb * row_blocks;
   if (c >= e.n) return;
   const int64_t wide = KIND == kDGated ? 2 * e.n : e.n, end = (blk + 1) * 32 < rows ? (blk + 1) * 32 : rows;
   float s0[V] = {}, s1[V] = {};
@@ -179,10 +180,11 @@ template <int KIND, int OUT>
 int launch_dz(const Epi& e, int64_t rows, cudaStream_t stream) {
   const bool vec = e.n % 4 == 0 && e.out_sr % 4 == 0 &&
                    ((reinterpret_cast<uintptr_t>(e.saved) | reinterpret_cast<uintptr_t>(e.out)) & 15) == 0;
-  const int64_t per = vec ? 512 : 128;
-  const dim3 grid((unsigned)((rows + 31) / 32), (unsigned)((e.n + per - 1) / per));
-  if (vec) launch_pdl(k_dz<KIND, OUT, 4>, grid, dim3(128), 0, stream, e, rows);
-  else launch_pdl(k_dz<KIND, OUT, 1>, grid, dim3(128), 0, stream, e, rows);
+  // one axis of blocks: the second one ends at 65535, which is 8.4 M columns in ranges of 128
+  const int64_t per = vec ? 512 : 128, row_blocks = (rows + 31) / 32, blocks = row_blocks * ((e.n + per - 1) / per);
+  SF_REQUIRE(blocks <= 0x7fffffff, "dz: %lld x %lld elements", (long long)rows, (long long)e.n);
+  if (vec) launch_pdl(k_dz<KIND, OUT, 4>, dim3((unsigned)blocks), dim3(128), 0, stream, e, rows, (unsigned)row_blocks);
+  else launch_pdl(k_dz<KIND, OUT, 1>, dim3((unsigned)blocks), dim3(128), 0, stream, e, rows, (unsigned)row_blocks);
   count_launch();
   return check_launch("dz");
 }

@@ -88,3 +88,23 @@ def test_a_transition_of_no_rows(dtype):
   assert x.grad.shape == x.shape
   for p in (lw, lb, w1, w2):
     assert p.grad.shape == p.shape and not p.grad.any()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("n", [(1 << 16) * 128 + 3, (1 << 16) * 512 + 4])
+def test_gradients_of_more_columns_than_a_grid_axis_has_blocks(n, gated):
+  """dz from saved pre-activations, in ranges of 128 columns (n odd) and of 512.  One row: dbias is dz before its rounding,
+  dy silu'(z) (2^-20 of the activation's terms, one product)."""
+  wide = 2 * n if gated else n
+  x, w = rnd(1, 1, 2).to(BF), torch.zeros(wide, 2, dtype=BF, device="cuda")
+  saved = torch.linspace(-6, 6, wide, device="cuda")[None].contiguous()
+  dy, b = torch.ones(1, n, dtype=BF, device="cuda"), torch.zeros(wide, device="cuda")
+  fn = ops.gated_linear_backward if gated else ops.linear_act_backward
+  got = fn(dy, x, w, b, activation="silu", saved=saved, need_dx=False, need_dwt=False)[2]
+  z, s = saved[0, :n], torch.sigmoid(saved[0, :n])
+  want = s * (1 + z * (1 - s)) * (saved[0, n:] if gated else 1.0)
+  # against fp32 arithmetic of the same formula: a few roundings of terms that are at most 1 + |z| (times |up|)
+  tol = 2.0 ** -18 * (1 + z.abs()) * (saved[0, n:].abs() if gated else 1.0) + 2.0 ** -30
+  assert bool(((got[:n] - want).abs() <= tol).all())
+  if gated:
+    assert bool(((got[n:] - z * s).abs() <= 2.0 ** -18 * z.abs() + 2.0 ** -30).all())

@@ -303,6 +303,8 @@ int sf_pair_sparse_linear(int dtype, const void* x, const float* w, const void* 
  * dw_sn, dw_sk; y, residual, dy [rows][n]; dx [rows][k] contiguous; y contiguous; bias, dbias [N] fp32.
  * saved [rows][N] fp32: the forward call writes the pre-activations x W^T + bias there when it is not
  * null; a backward call reads them from there, or computes them again from x and wt when it is null.
+ * dbias may be asked for without a bias; pass saved = null then, as only a layer with a bias saves pre-activations
+ * that were summed in the short runs which a sum over many rows needs (else dbias is off by 1.1e-9 k of itself).
  * y may alias residual; no other output may alias anything.  rows == 0 is allowed (dwt and dbias are
  * then zero).  fp32 tensors are computed to fp32 accuracy: each operand is split into three bf16
  * terms whose six largest products run on the tensor cores, so an infinite or NaN operand makes the

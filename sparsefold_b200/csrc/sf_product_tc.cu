@@ -141,7 +141,8 @@ int product_tc(const Operand& a, const Operand& b, const Operand* b2, const Epi&
   // Segments of 512 for fp32 operands, and for the pre-activations that dbias comes from: the accumulator truncates
   // (1.1e-9 of a value per column), and a sum over the rows does not average that away (K = 2048, gated silu, dbias
   // against fp64: 2.2e-6 in segments of 2048, 5.1e-7 in these; 2000 rows of 4096 columns 33 us either way).
-  p.seg_kb = p.pairs > 1 || (e.bias && (e.saved || e.colpart)) ? 8 : p.nkb;
+  // (dbias may be asked for without a bias: colpart; saved ones only serve it where the layer has one)
+  p.seg_kb = p.pairs > 1 || e.colpart || (e.bias && e.saved) ? 8 : p.nkb;
   // a plain sum's K may be split over CTAs
   const bool plain = e.kind == kLinear && e.act == SF_POST_NONE && !e.bias && !e.aux && !e.saved;
   const Plan plan = plan_of(p.m, p.n, p.nkb, p.pairs, p.seg_kb, gated, b.k_major, plain, sms);

@@ -1,9 +1,12 @@
 """linear_act, gated_linear and their gradients where a single call's agreement with the formula shows too little:
 repeated calls, forms that the C ABI allows, values at the ends of the activations, errors of whole tensors."""
+import ctypes as C
+
 import pytest
 import torch
 
-from sparsefold_b200 import _native, ops, training
+from sparsefold_b200 import _native as N
+from sparsefold_b200 import ops, training
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -13,9 +16,9 @@ BF, F32 = torch.bfloat16, torch.float32
 def _device():
   if not torch.cuda.is_available():
     pytest.skip("no CUDA device")
-  _native.check(_native.load().sf_device_check(), "sf_device_check")
+  N.check(N.load().sf_device_check(), "sf_device_check")
   yield
-  assert _native.device_status() == 0
+  assert N.device_status() == 0
 
 
 def rnd(seed, *s):
@@ -108,3 +111,25 @@ def test_gradients_of_more_columns_than_a_grid_axis_has_blocks(n, gated):
   assert bool(((got[:n] - want).abs() <= tol).all())
   if gated:
     assert bool(((got[n:] - z * s).abs() <= 2.0 ** -18 * z.abs() + 2.0 ** -30).all())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k", [2048, 8192])
+def test_bias_gradient_without_a_bias(k, gated):
+  """The C ABI gives dbias without a bias too, to the same accuracy: z short by at most 512 * 1.1e-9 = 5.6e-7 of itself,
+  whose part in dbias is at most 1.5 of that, and roundings that average out over the rows: 2^-20 of its norm."""
+  rows, n = 2000, 72
+  wide = 2 * n if gated else n
+  x, w, dy = rnd(1, rows, k).to(BF), (rnd(2, wide, k) / k ** 0.5).to(BF), rnd(3, rows, n).to(BF)
+  db = torch.empty(wide, device="cuda")
+  op = N.SF_OP_GATED_LINEAR_BACKWARD if gated else N.SF_OP_LINEAR_ACT_BACKWARD
+  a = N.LinearArgs(dtype=N.SF_BF16, activation=N.ACTIVATIONS["silu"], rows=rows, k=k, n=n, x=x.data_ptr(), x_sr=k,
+                   wt=w.data_ptr(), w_sn=k, w_sk=1, dy=dy.data_ptr(), dy_sr=n, dbias=db.data_ptr())
+  need = N.load().sf_linear_act_workspace(C.byref(a), op)
+  ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+  N.call("sf_gated_linear_backward" if gated else "sf_linear_act_backward", C.byref(a), ws.data_ptr(), need,
+         torch.cuda.current_stream().cuda_stream)
+  z = (x.double() @ w.double().t()).requires_grad_(True)
+  y = torch.nn.functional.silu(z[:, :n]) * (z[:, n:] if gated else 1.0)
+  ref = torch.autograd.grad((y * dy.double()).sum(), z)[0].sum(0)
+  assert gap(db, ref) <= 2.0 ** -20

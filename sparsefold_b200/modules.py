@@ -16,6 +16,7 @@ modules do (backends/vecops/modules.py:88-94).
 from __future__ import annotations
 
 import functools
+import warnings
 import weakref
 
 import torch
@@ -37,9 +38,20 @@ def _tag(dtype: torch.dtype) -> str:
   return "f32" if dtype == torch.float32 else "bf16"
 
 
+def _warn_where_gradients_end(module, tensors) -> None:
+  """Only a TransitionBlock that ``trainable`` switched on passes gradients on; the other modules' outputs carry none,
+  and autograd would leave out what lies before them without a word."""
+  if getattr(module, "_sf_trainable", False) or not torch.is_grad_enabled():
+    return
+  if any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    warnings.warn(f"{type(module).__name__} runs forward only: its input requires a gradient, and none passes through it "
+                  "(use torch.no_grad() or detach() where none is wanted)", stacklevel=3)
+
+
 def _require_prepared(fn):
   @functools.wraps(fn)
   def wrapped(self, *args, **kwargs):
+    _warn_where_gradients_end(self, (*args, *kwargs.values()))
     if not getattr(self, "_native_prepared", False):
       raise RuntimeError("Native buffers are not prepared; call backends.prepare(model) after weight loading")
     dev = args[0].device if args and isinstance(args[0], torch.Tensor) else None
@@ -916,7 +928,7 @@ def trainable(module: torch.nn.Module, on: bool = True) -> list[torch.nn.Paramet
   ``training.transition`` on their parameters themselves (not on the packed copies), which get
   requires_grad, and pass gradients to their input.  Returns those parameters.  The other modules stay
   forward-only: their outputs carry no gradient, so in a stack a transition's parameters get one only from
-  what lies between it and the next of those.  ``on=False`` goes back to the fused forward kernel and packs
+  what lies between it and the next of those (which warns when its input requires a gradient).  ``on=False`` goes back to the fused forward kernel and packs
   the parameters as they are then for it."""
   params = []
   for m in module.modules():

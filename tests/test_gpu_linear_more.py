@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from sparsefold_b200 import _native as N
-from sparsefold_b200 import ops, training
+from sparsefold_b200 import modules, ops, synth, training
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -133,3 +133,25 @@ def test_bias_gradient_without_a_bias(k, gated):
   y = torch.nn.functional.silu(z[:, :n]) * (z[:, n:] if gated else 1.0)
   ref = torch.autograd.grad((y * dy.double()).sum(), z)[0].sum(0)
   assert gap(db, ref) <= 2.0 ** -20
+
+
+def test_a_stack_trains_its_last_transitions_and_says_so():
+  """Two Pairformer blocks: gradients reach the transitions behind the last forward-only module of each track, and the
+  first block's, which feed such modules, stay without one; the second block's modules warn of it."""
+  blocks = torch.nn.ModuleList(modules.PairFormerIteration() for _ in range(2))
+  for i, b in enumerate(blocks):
+    synth.init_params(b, seed=i)
+  modules.prepare(blocks)
+  blocks = blocks.cuda()
+  modules.trainable(blocks)
+  pair, single = rnd(1, 24, 24, 128).to(BF), rnd(2, 24, 384).to(BF)
+  mask = torch.ones(24, dtype=torch.bool, device="cuda")
+  with pytest.warns(UserWarning, match="runs forward only"):
+    for b in blocks:
+      pair, single = b(pair, seq_mask=mask, single_act=single)
+  (pair.float().square().sum() + single.float().square().sum()).backward()
+  for i, b in enumerate(blocks):
+    for t in (b.pair_transition, b.single_act_update.single_transition):
+      for p in (t.input_layer_norm.weight, t.input_layer_norm.bias, t.transition1.weight, t.transition2.weight):
+        assert (p.grad is None) == (i == 0)
+        assert i == 0 or (bool(torch.isfinite(p.grad).all()) and bool(p.grad.any()))

@@ -128,3 +128,26 @@ def test_layer_norm_of_no_rows(monkeypatch):
   w = torch.ones(8).as_subclass(OnOne)
   for shape in ((0, 8), (3, 0, 8)):
     assert ops.layer_norm(torch.zeros(shape).as_subclass(OnOne), w, w).shape == shape
+
+
+def test_a_forward_only_module_warns_where_a_gradient_ends(recwarn):
+  class Forward(modules.B200Module, torch.nn.Module):
+    _native_prepared = True
+
+    @modules._require_prepared
+    def forward(self, x, *, residual=None):
+      return x.detach()
+
+  m, x = Forward(), torch.zeros(3)
+  m(x)
+  m(x, residual=torch.zeros(3))
+  with torch.no_grad():
+    m(torch.zeros(3, requires_grad=True))
+  m._sf_trainable = True
+  m(torch.zeros(3, requires_grad=True))
+  assert not recwarn.list
+  m._sf_trainable = False
+  with pytest.warns(UserWarning, match="Forward runs forward only"):
+    m(torch.zeros(3, requires_grad=True))
+  with pytest.warns(UserWarning, match="none passes through"):
+    m(x, residual=torch.zeros(3, requires_grad=True))

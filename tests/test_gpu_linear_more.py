@@ -155,3 +155,62 @@ def test_a_stack_trains_its_last_transitions_and_says_so():
       for p in (t.input_layer_norm.weight, t.input_layer_norm.bias, t.transition1.weight, t.transition2.weight):
         assert (p.grad is None) == (i == 0)
         assert i == 0 or (bool(torch.isfinite(p.grad).all()) and bool(p.grad.any()))
+
+
+# ---- errors of whole tensors ------------------------------------------------------------------------------
+# Elementwise bounds over all magnitudes are far above what random signs leave, so that a term or a row may be missing
+# within them.  Norm of the error over norm of the result, instead, with e = 6.8e-7 for one fp32 product: a sum of 512
+# columns is short by at most 5.6e-7 of itself, the dropped terms are 2^-23.  An activation changes by at most 1.5 times
+# what its argument does; a gated value has two factors; gradients are products of what dz carries, with their own e.
+# bf16: one rounding to nearest is 2^-9 / sqrt(3) to 2^-8 / sqrt(3) of a value over its binade, 0.0017 over them all
+# and below 2^-9 = 0.00195; two in a row (dz, the result) below sqrt(2) 2^-9.
+E32 = 6.8e-7
+SIZES = [(500, 512, 520), (2000, 4096, 264), (8000, 768, 128), (1000, 8192, 72), (600, 700, 4000), (4700, 1100, 600),
+         (9401, 75, 601), (19000, 64, 40), (40, 4096, 2056), (33, 700, 96), (65, 2056, 1030)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kn", [False, True])
+@pytest.mark.parametrize("rows,k,n", SIZES)
+def test_errors_of_whole_tensors(rows, k, n, kn, gated, dtype):
+  wide = 2 * n if gated else n
+  x, dy, b = rnd(1, rows, k).to(dtype), rnd(2, rows, n).to(dtype), 0.5 * rnd(3, wide)
+  w = (rnd(4, k, wide) / k ** 0.5).to(dtype).t() if kn else (rnd(4, wide, k) / k ** 0.5).to(dtype)
+  fw, bw = (ops.gated_linear, ops.gated_linear_backward) if gated else (ops.linear_act, ops.linear_act_backward)
+  y, saved = fw(x, w, b, activation="silu", save=True)
+  z = (x.double() @ w.double().t() + b.double()).requires_grad_(True)
+  ref = torch.nn.functional.silu(z[:, :n]) * (z[:, n:] if gated else 1.0)
+  dz = torch.autograd.grad((ref * dy.double()).sum(), z)[0]
+  ref = ref.detach()
+  one, two = (2.0 ** -9, 2.0 ** -8.5) if dtype == BF else ((2.5 if gated else 1.5) * E32, (3.5 if gated else 2.5) * E32)
+  assert gap(y, ref) <= one
+  for s in {id(saved): saved, 0: None}.values():
+    dx, dw, db = bw(dy, x, w, b, activation="silu", saved=s)
+    assert gap(dx, dz @ w.double()) <= two
+    assert gap(dw, dz.t() @ x.double()) <= two
+    assert gap(db, dz.sum(0)) <= (3.5 if gated else 2.5) * E32      # fp32 in both types, from unrounded dz
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,k,n", [(19000, 64, 40), (9401, 75, 601), (4700, 1100, 600), (2047, 139, 128), (513, 96, 384)])
+def test_the_last_rows_count(rows, k, n, dtype):
+  """dy is zero but in the rows behind the last whole 64, then in the last row alone, then in the rows around every
+  512th (where sums of runs meet): dW and dbias have to come from those rows."""
+  x, w, b = rnd(1, rows, k).to(dtype), (rnd(2, n, k) / k ** 0.5).to(dtype), rnd(3, n)
+  full = rnd(4, rows, n).to(dtype)
+  z = x.double() @ w.double().t() + b.double()
+  s = torch.sigmoid(z)
+  da = s * (1 + z * (1 - s))
+  index = torch.arange(rows, device="cuda")
+  for keep in (index >= rows // 64 * 64, index == rows - 1, (index + 2) % 512 < 4):
+    dy = full * keep[:, None].to(dtype)
+    dx, dw, db = ops.linear_act_backward(dy, x, w, b, activation="silu")
+    if not bool(keep.any()):
+      assert not (dx.any() or dw.any() or db.any())
+      continue
+    dz = dy.double() * da
+    assert gap(dw, dz.t() @ x.double()) <= (2.0 ** -8.5 if dtype == BF else 2.5 * E32)
+    assert gap(dx, dz @ w.double()) <= (2.0 ** -8.5 if dtype == BF else 2.5 * E32)
+    assert gap(db, dz.sum(0)) <= 2.5 * E32 + 2.0 ** -20 * (dtype == BF)     # the fast activation's 2^-21, few rows
+    assert not dx[~keep].any()

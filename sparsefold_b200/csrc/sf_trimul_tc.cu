@@ -256,7 +256,20 @@ int num_sms() {
 
 // cuTensorMapEncodeTiled resolved through the runtime, so the library does not
 // link libcuda directly (it loads on machines without a driver).
+// It needs a current context, which the runtime binds to a thread at its first call there: a thread whose first CUDA call
+// would be this one (an autograd worker on its first backward pass) asks for its device's here.
 EncodeTiledFn tensor_map_encoder() {
+  static thread_local bool bound = false;
+  if (!bound) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) {
+      set_error("no CUDA context for the tensor maps: %s", cudaGetErrorString(e));
+      return nullptr;
+    }
+    bound = true;
+  }
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* p = nullptr;

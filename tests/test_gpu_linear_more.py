@@ -1,6 +1,7 @@
 """linear_act, gated_linear and their gradients where a single call's agreement with the formula shows too little:
 repeated calls, forms that the C ABI allows, values at the ends of the activations, errors of whole tensors."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -214,3 +215,18 @@ def test_the_last_rows_count(rows, k, n, dtype):
     assert gap(dx, dz @ w.double()) <= (2.0 ** -8.5 if dtype == BF else 2.5 * E32)
     assert gap(db, dz.sum(0)) <= 2.5 * E32 + 2.0 ** -20 * (dtype == BF)     # the fast activation's 2^-21, few rows
     assert not dx[~keep].any()
+
+
+@pytest.mark.parametrize("rows", [4, 70, 9400])
+def test_the_first_call_of_a_thread(rows):
+  """A thread that has made no CUDA call yet, as an autograd worker on its first backward pass, has no current context
+  until the runtime binds one; the tensor maps need it."""
+  x, w, dy = rnd(1, rows, 64).to(BF), rnd(2, 96, 64).to(BF), rnd(3, rows, 96).to(BF)
+  want = ops.linear_act_backward(dy, x, w)[:2]
+  got = []
+  for call in (lambda: got.append(ops.linear_act(x, w)), lambda: got.extend(ops.linear_act_backward(dy, x, w)[:2])):
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+  assert len(got) == 3 and torch.equal(got[0], ops.linear_act(x, w))
+  assert torch.equal(got[1], want[0]) and torch.equal(got[2], want[1])

@@ -230,3 +230,137 @@ def test_the_first_call_of_a_thread(rows):
     t.join()
   assert len(got) == 3 and torch.equal(got[0], ops.linear_act(x, w))
   assert torch.equal(got[1], want[0]) and torch.equal(got[2], want[1])
+
+
+# ---- calls that the documentation allows ------------------------------------------------------------------
+ROWS = [1, 4, 20, 140, 9400]     # dot products, tiles with and without a staged epilogue, clusters of two
+
+
+def padded(t, pad):
+  """t as a view of wider rows, NaN behind each."""
+  room = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), dtype=t.dtype, device=t.device)
+  room[:, :t.shape[1]] = t
+  return room[:, :t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("pad", [8, 3])
+@pytest.mark.parametrize("k,n", [(72, 600), (1100, 77)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_strided_rows_of_dy_and_residual(rows, k, n, pad, dtype):
+  """The same values in wider rows, which TMA reads (pad 8) or plain loads do: the same bits."""
+  x, res = rnd(1, rows, k).to(dtype), rnd(2, rows, n).to(dtype)
+  for gated in (False, True):
+    wide = 2 * n if gated else n
+    w, b, dy = (rnd(3, wide, k) / k ** 0.5).to(dtype), rnd(4, wide), rnd(5, rows, n).to(dtype)
+    fw, bw = (ops.gated_linear, ops.gated_linear_backward) if gated else (ops.linear_act, ops.linear_act_backward)
+    saved = fw(x, w, b, activation="gelu", save=True)[1]
+    for s in {id(saved): saved, 0: None}.values():
+      for act in ("gelu", None):      # without an activation dy is itself the products' operand
+        want = bw(dy, x, w, b, activation=act, saved=s)
+        for u, v in zip(bw(padded(dy, pad), x, w, b, activation=act, saved=s), want):
+          assert torch.equal(u, v)
+  w, b = w[:n].contiguous(), b[:n].contiguous()
+  for act in ("gelu", None):
+    want = ops.linear_act(x, w, b, activation=act, residual=res, save=True)
+    got = ops.linear_act(x, w, b, activation=act, residual=padded(res, pad), save=True)
+    assert torch.equal(got[0], want[0]) and (want[1] is None or torch.equal(got[1], want[1]))
+    assert gap(want[0], res.double() + ops.linear_act(x.double().float(), w.float(), b, activation=act).double()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("n", [600, 77])
+@pytest.mark.parametrize("rows", ROWS)
+def test_y_in_the_place_of_the_residual(rows, n, dtype):
+  """The C ABI allows it; every element of the residual is read before it is written."""
+  k = 72
+  x, w, b, res = rnd(1, rows, k).to(dtype), (rnd(2, n, k) / k ** 0.5).to(dtype), rnd(3, n), rnd(4, rows, n).to(dtype)
+  want = ops.linear_act(x, w, b, activation="silu", residual=res)
+  a = N.LinearArgs(dtype=N.SF_BF16 if dtype == BF else N.SF_F32, activation=N.ACTIVATIONS["silu"], rows=rows, k=k, n=n,
+                   x=x.data_ptr(), x_sr=k, wt=w.data_ptr(), w_sn=k, w_sk=1, bias=b.data_ptr(), residual=res.data_ptr(),
+                   r_sr=n, y=res.data_ptr())
+  need = N.load().sf_linear_act_workspace(C.byref(a), N.SF_OP_LINEAR_ACT)
+  ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+  N.call("sf_linear_act", C.byref(a), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+  assert torch.equal(res, want)
+
+
+def test_bf16_activations_with_fp32_parameters():
+  """A block that holds fp32 parameters and meets bf16 activations: fp32 gradients of the bf16 weights' products.  Three
+  layers forward and back, each with roundings of 2^-9 on average: 2^-7 of each gradient's norm."""
+  blk = modules.TransitionBlock(64, 2)
+  p = synth.init_params(blk, seed=3)
+  modules.prepare(blk)
+  blk = blk.cuda()
+  params = modules.trainable(blk)
+  x, dy = rnd(8, 5, 21, 64).to(BF).requires_grad_(True), rnd(9, 5, 21, 64).to(BF)
+  y = blk(x)
+  assert y.dtype == BF
+  y.backward(dy)
+  assert x.grad.dtype == BF and all(q.dtype == q.grad.dtype == F32 for q in params)
+  r = {k: v.cuda().double().requires_grad_(True) for k, v in p.items()}
+  xr = x.detach().double().requires_grad_(True)
+  n = torch.nn.functional.layer_norm(xr, (64,), r["input_layer_norm.weight"], r["input_layer_norm.bias"], 1e-5)
+  gate, up = (n @ r["transition1.weight"]).chunk(2, -1)
+  (xr + (torch.nn.functional.silu(gate) * up) @ r["transition2.weight"]).backward(dy.double())
+  assert gap(x.grad, xr.grad) <= 2.0 ** -7
+  for q, name in zip(params, ("input_layer_norm.weight", "input_layer_norm.bias", "transition1.weight", "transition2.weight")):
+    assert gap(q.grad, r[name].grad) <= 2.0 ** -7
+
+
+def test_two_threads():
+  """Calls of two threads on streams of their own, interleaved: the bits of the same calls alone."""
+  def work(seed, rows, k, n):
+    x, w, b, dy = rnd(seed, rows, k).to(BF), rnd(seed + 1, 2 * n, k).to(BF), rnd(seed + 2, 2 * n), rnd(seed + 3, rows, n).to(BF)
+    return lambda: (ops.gated_linear(x, w, b), *ops.gated_linear_backward(dy, x, w, b),
+                    ops.clip_grad_norm([x.clone(), dy.clone()], 1.0), *ops.layer_norm_backward(x, x))
+  jobs = [work(1, 4700, 136, 600), work(11, 9, 1200, 264)]
+  want = [job() for job in jobs]
+  torch.cuda.synchronize()
+  wrong = []
+
+  def run(job, expect):
+    try:
+      with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):
+          for u, v in zip(job(), expect):
+            if v is not None and not torch.equal(u, v):
+              wrong.append("other bits")
+    except Exception as e:          # a failure in a thread would be lost
+      wrong.append(repr(e))
+
+  threads = [threading.Thread(target=run, args=a) for a in zip(jobs, want)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert not wrong
+
+
+def test_a_captured_training_pass():
+  """Warm-up and capture on one side stream, no eager graph of the leaves alive: replays follow their inputs."""
+  x, lw, lb = rnd(1, 70, 64).to(BF), 1 + 0.1 * rnd(2, 64), 0.1 * rnd(3, 64)
+  w1, w2, dy = (rnd(4, 256, 64) / 8).to(BF), (rnd(5, 64, 128) / 11).to(BF), rnd(6, 70, 64).to(BF)
+  leaves = [t.requires_grad_(True) for t in (x, lw, lb, w1, w2)]
+
+  def step():
+    y = training.transition(*leaves)
+    return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    step()
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph, stream=side):
+    got = step()
+  with torch.no_grad():
+    x.copy_(rnd(7, 70, 64))
+    w1.mul_(-0.5)
+    dy.mul_(2.0)
+  graph.replay()
+  torch.cuda.synchronize()
+  replayed = [t.clone() for t in got]
+  for u, v in zip(replayed, step()):
+    assert torch.equal(u, v)

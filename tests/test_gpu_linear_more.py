@@ -364,3 +364,81 @@ def test_a_captured_training_pass():
   replayed = [t.clone() for t in got]
   for u, v in zip(replayed, step()):
     assert torch.equal(u, v)
+
+
+class Room:
+  """Outputs of the C ABI inside larger buffers of a known byte, at odd offsets: what lies around them stays as it was."""
+
+  def __init__(self):
+    self.all = []
+
+  def take(self, rows, cols, dtype, pad=0, offset=1):
+    buf = torch.full(((rows * (cols + pad) + 64 + offset) * dtype.itemsize,), 0xA5, dtype=torch.uint8, device="cuda").view(dtype)
+    view = buf[32 + offset:32 + offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+    self.all.append((buf, buf.clone(), view.storage_offset(), rows, cols, cols + pad))
+    return view
+
+  def check(self):
+    for buf, before, at, rows, cols, pitch in self.all:
+      outside = torch.ones(buf.numel(), dtype=torch.bool, device="cuda")
+      outside.as_strided((rows, cols), (pitch, 1), at).fill_(False)
+      size = {2: torch.int16, 4: torch.int32, 1: torch.uint8}[buf.element_size()]
+      assert torch.equal(buf.view(size)[outside], before.view(size)[outside])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kn", [False, True])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("rows,k,n", [(1, 72, 40), (7, 33, 5), (20, 40, 77), (140, 72, 56), (301, 1100, 130), (4700, 136, 601)])
+def test_nothing_else_is_written(rows, k, n, offset, kn, gated, dtype):
+  """Both directions through the C ABI: outputs without alignment, dwt in rows wider than its own, a workspace of exactly
+  the bytes asked for; the values are those of the Python calls, the surroundings stay."""
+  wide = 2 * n if gated else n
+  x, dy, b = rnd(1, rows, k).to(dtype), rnd(2, rows, n).to(dtype), rnd(3, wide)
+  w = (rnd(4, k, wide) / 9).to(dtype).t() if kn else (rnd(4, wide, k) / 9).to(dtype)
+  fw, bw = (ops.gated_linear, ops.gated_linear_backward) if gated else (ops.linear_act, ops.linear_act_backward)
+  want_y, want_saved = fw(x, w, b, activation="silu", save=True)
+  want = bw(dy, x, w, b, activation="silu", saved=None)
+  room = Room()
+  y, saved, dx = (room.take(rows, c, t, offset=offset) for c, t in ((n, dtype), (wide, F32), (k, dtype)))
+  dwt, db = room.take(*((k, wide) if kn else (wide, k)), dtype, pad=3 + 5 * (offset == 0), offset=offset), room.take(1, wide, F32)
+  sn, sk = (1, wide) if kn else (k, 1)
+  dn, dk = (1, dwt.stride(0)) if kn else (dwt.stride(0), 1)
+
+  def call(name, op, **more):
+    a = N.LinearArgs(dtype=N.SF_BF16 if dtype == BF else N.SF_F32, activation=N.ACTIVATIONS["silu"], rows=rows, k=k, n=n,
+                     x=x.data_ptr(), x_sr=k, wt=w.data_ptr(), w_sn=sn, w_sk=sk, bias=b.data_ptr(), **more)
+    need = N.load().sf_linear_act_workspace(C.byref(a), op)
+    ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    N.call(name, C.byref(a), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert bool((ws[need:] == 0x5A).all())
+
+  form = "sf_gated_linear" if gated else "sf_linear_act"
+  forward = N.SF_OP_GATED_LINEAR if gated else N.SF_OP_LINEAR_ACT
+  keep = want_saved is not None
+  call(form, forward, y=y.data_ptr(), saved=saved.data_ptr() if keep else None)
+  assert torch.equal(y, want_y) and (not keep or torch.equal(saved, want_saved))
+  back = N.SF_OP_GATED_LINEAR_BACKWARD if gated else N.SF_OP_LINEAR_ACT_BACKWARD
+  call(form + "_backward", back, dy=dy.data_ptr(), dy_sr=n, dx=dx.data_ptr(), dwt=dwt.data_ptr(), dw_sn=dn, dw_sk=dk,
+       dbias=db.data_ptr())
+  assert torch.equal(dx, want[0]) and torch.equal(dwt.t() if kn else dwt, want[1]) and torch.equal(db[0], want[2])
+  room.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("sums", [False, True])
+@pytest.mark.parametrize("rows,cols", [(5, 24), (3000, 128), (700, 267), (100, 768), (33, 4096), (40, 9000)])
+def test_dx_in_the_place_of_dy(rows, cols, sums, dtype):
+  """The C ABI of the LayerNorm gradient allows it."""
+  x, dy, w, b = rnd(1, rows, cols).to(dtype), rnd(2, rows, cols).to(dtype), 1 + 0.1 * rnd(3, cols), rnd(4, cols)
+  want = ops.layer_norm_backward(dy, x, w, b, need_dweight=sums, need_dbias=sums)
+  dw, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+  need = N.load().sf_layernorm_backward_workspace(rows, cols)
+  ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+  N.call("sf_layernorm_backward", N.SF_BF16 if dtype == BF else N.SF_F32, dy.data_ptr(), x.data_ptr(), w.data_ptr(),
+         dy.data_ptr(), dw.data_ptr() if sums else None, db.data_ptr() if sums else None, rows, cols, 1e-5, ws.data_ptr(),
+         need, torch.cuda.current_stream().cuda_stream)
+  assert torch.equal(dy, want[0]) and bool((ws[need:] == 0x5A).all())
+  if sums:
+    assert torch.equal(dw, want[1]) and torch.equal(db, want[2])

@@ -5,6 +5,9 @@
 //      again;  no pass at all for a linear layer without activation, where dz = dy;
 //   2. dx = dz W;   3. dW = dz^T x (or its transpose, whichever way dwt is laid out);
 //   4. dbias: column sums of dz before its rounding.
+// dz is held in the call's type: a bf16 dz is one operand of one product, as x and W are, where an unrounded one would be
+// two terms and twice the products of 2 and 3 (8192 x 2048 -> 2 x 8192: 1650 GFLOP in all, two thirds of it theirs).  The
+// rounding's 2^-9 on average adds to that of the result: 0.0023 of a bf16 gradient's norm against fp64, 0.0017 without it.
 #include <type_traits>
 
 #include "sf_linear_grad.cuh"

@@ -9,7 +9,7 @@
 // another issues tcgen05.mma (M 128, N = bn, K 16) into one of two TMEM accumulators of up to 256 columns; 8 or 16
 // warps drain the other one (thread = row).  Few tiles and a deep K: the K loop is split over CTAs, fp32 partials
 // summed in order by k_sums.  Waits that are long as a rule are suspended and the ring's slots counted
-// without divisions: polling and dividing threads took 20 % of the products' time (454 -> 360 us at that size).
+// without divisions: polling and dividing threads took 20 % of the products' time (16384 x 4096 x 4096: 454 -> 360 us).
 #pragma once
 
 #include "sf_linear_grad.cuh"
@@ -32,7 +32,7 @@ constexpr int GROUP_M = 12;                         // row tiles that share B ti
 // CTAS = 2: a cluster of two CTAs computes 256 x bn tiles with cta_group::2 MMAs.  Each CTA loads its 128 rows
 // of A and half of B's rows, so a 256 x 256 tile moves 2 x 32 KB per 64-deep step instead of 2 x 48 KB: the L2
 // reads and the shared-memory reads of B halve (16384 x 4096 x 4096 bf16: 430 us with single CTAs, 664 with both
-// operands M/N-major; 360 and 390 us in pairs, where the library product takes 345 and 350).
+// operands M/N-major; 353 and 385 us in pairs, where the library product takes 346 and 357; tensor pipe 90 % active).
 
 // The six term products of two split fp32 operands, smallest first, as nibbles (a plane, b plane).
 constexpr uint32_t kPairA = 0x001102u, kPairB = 0x010120u;   // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
@@ -214,7 +214,8 @@ __device__ __forceinline__ pair_t sigmoid2(pair_t z) {
   return rcp2(add2(ex2_2(mul2(z, pk1(-1.4426950408889634f))), pk1(1.0f)));
 }
 // Phi(z) and exp(-z^2 / 2) as normal_cdf<true>: q is chosen by the sign of z, not formed as 1 - (1 - q), which would
-// lose it in the negative tail (4 % of gelu at z = -5, all of it at -6).
+// lose it in the negative tail (4 % of gelu at z = -5, all of it at -6).  65536 x 128 -> 2 x 1024: forward 76 us, backward
+// 239 (75 and 232 with five terms and that loss).
 __device__ __forceinline__ void cdf2(pair_t z, pair_t& cdf, pair_t& e) {
   e = ex2_2(mul2(mul2(z, z), pk1(-0.72134752044448170f)));
   const pair_t t = rcp2(fma2(pk1(kTailC), z & 0x7FFFFFFF7FFFFFFFull, pk1(1.0f)));

@@ -380,8 +380,9 @@ def pair_sparse_linear(x: torch.Tensor, w_kc: torch.Tensor, residual=None) -> to
 # linear layers with gradients, the LayerNorm gradient, gradient clipping
 # ---------------------------------------------------------------------------
 # A forward call with save=True keeps the fp32 pre-activations only above this input width.  Up to it the
-# backward computes them again: 2 k flop at the tensor cores' rate against 8 bytes (written and read back)
-# at the memory's, which meet near k = 1000.
+# backward computes them again: for many bf16 rows 2 k flop at the tensor cores' rate against 8 bytes (written and
+# read back) at the memory's meet near k = 1000.  One rule for all: fp32 operands (six products, k = 170) and few rows
+# (pre-activations that stay in L2; 3840 x 768 x 768 spends 17 us on the second product) would gain from saving earlier.
 SAVE_ABOVE_K = 1024
 
 

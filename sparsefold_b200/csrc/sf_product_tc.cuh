@@ -478,7 +478,9 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
-// Waits until at most `left` (0 or 1) of the warp's last stores still read their buffers.
+// Waits until at most `left` (0 or 1) of the warp's last stores still read their buffers.  One left over means the other
+// buffer's only if every use of a buffer commits a group: warps without a row in a tile commit an empty one (without it
+// they overwrote what the tile before still had to store, seen where the stores are the bound: 12346 x 8 -> 4072).
 __device__ __forceinline__ void free_slot(int left, int lane) {
   if (lane == 0) {
     if (left == 0) tc::bulk_wait_read0();
@@ -541,8 +543,8 @@ __device__ __forceinline__ void store_f32(const CUtensorMap* map, float* dst, in
   if (tma) {
     tc::fence_proxy_async();
     __syncwarp();
-    if (lane == 0 && rows > 0) {
-      tc::tma_store_3d(map, buf, c, row0, z);
+    if (lane == 0) {
+      if (rows > 0) tc::tma_store_3d(map, buf, c, row0, z);
       tc::bulk_commit();
     }
   } else {
@@ -765,9 +767,11 @@ __device__ __forceinline__ void staged_epilogue(const Params& p, const Maps& tm,
       if (p.vec_out) {
         tc::fence_proxy_async();
         __syncwarp();
-        if (lane == 0 && rows > 0) {
-          tc::tma_store_3d(&tm.out, out_buf, c0 + c, row0, split);
-          if (KIND == kDGated) tc::tma_store_3d(&tm.out2, out_buf + SLOT, c0 + c, row0, split);
+        if (lane == 0) {
+          if (rows > 0) {
+            tc::tma_store_3d(&tm.out, out_buf, c0 + c, row0, split);
+            if (KIND == kDGated) tc::tma_store_3d(&tm.out2, out_buf + SLOT, c0 + c, row0, split);
+          }
           tc::bulk_commit();
         }
       } else {

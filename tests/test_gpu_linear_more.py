@@ -51,6 +51,25 @@ def test_pairs_of_ctas_give_the_same_bits_every_time(rows, k, n, kn):
       assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,k,n", [(12346, 8, 4072), (16397, 16, 2048), (2976, 104, 4840), (9610, 40, 3320)])
+def test_large_outputs_of_few_columns_give_the_same_bits_every_time(rows, k, n, dtype):
+  """Bound by the stores, with warps that have no row in the last row tile: what the tile before it has staged must leave
+  its buffer first.  Twenty calls of each form; a wrong buffer is 1024 elements of another tile."""
+  x, w, b, res = rnd(1, rows, k).to(dtype), (rnd(2, n, k) / k ** 0.5).to(dtype), rnd(3, n), rnd(4, rows, n).to(dtype)
+  dy, half = rnd(5, rows, k).to(dtype), n // 2
+  z = x.double() @ w.double().t()
+  calls = [(lambda: ops.linear_act(x, w), z),
+           (lambda: ops.linear_act(x, w, b, activation="sigmoid", residual=res), torch.sigmoid(z + b.double()) + res.double()),
+           (lambda: ops.gated_linear(x, w), torch.nn.functional.silu(z[:, :half]) * z[:, half:]),
+           (lambda: ops.linear_act_backward(dy, res, w.t(), need_dwt=False)[0], dy.double() @ w.double().t())]
+  for call, ref in calls:
+    first = call()
+    assert gap(first, ref) <= (2.0 ** -9 * 1.05 if dtype == BF else 3 * 6.8e-7)
+    for _ in range(20):
+      assert torch.equal(call(), first)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows,k,n", [(4, 16, 48), (20, 16, 48), (20, 4096, 4104), (200, 72, 72), (200, 1200, 77), (9400, 72, 600)])
 def test_gelu_keeps_its_tail(rows, k, n, dtype):

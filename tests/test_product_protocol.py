@@ -136,6 +136,48 @@ def test_the_model_catches_planted_mistakes():
   assert caught == 20
 
 
+def stage(tiles, seed, committed=True):
+  """One warp's output buffers over several tiles (rows of its own in a tile or none, chunks per tile): two buffers in turn,
+  a wait for all but the last group before each use, a store that reads its buffer some time after its commit."""
+  rng = random.Random(seed)
+  groups, turn = [], 0              # committed groups in order: [buffer that is read, or None for an empty one; done]
+  for tile, (rows, chunks) in enumerate(tiles):
+    for _ in range(chunks):
+      for g in groups[:-1]:
+        g[1] = True                 # the wait: all but the last group have read their buffers
+      buf, turn = turn & 1, turn + 1
+      assert not any(g[0] == buf and not g[1] for g in groups), f"tile {tile}: a store still reads buffer {buf}"
+      if rows or committed:
+        groups.append([buf if rows else None, not rows])
+      late = [g for g in groups if not g[1]]
+      if late and rng.random() < 0.3:
+        late[0][1] = True           # the engine reads on
+
+
+def test_buffers_of_warps_without_rows():
+  """The last row tile leaves some warps without a row; the tile before it may still be on its way out."""
+  rng = random.Random(1)
+  for seed in range(200):
+    stage([(rng.random() < 0.6, rng.randint(0, 3)) for _ in range(30)], seed)
+  caught = 0
+  for seed in range(20):
+    try:
+      stage([(True, 2), (False, 2), (True, 2)] * 10, seed, committed=False)
+    except AssertionError:
+      caught += 1
+  assert caught == 20
+
+
+def test_every_use_of_a_buffer_commits_a_group():
+  text = re.sub(r"//[^\n]*", "", open(SOURCE).read())
+  at = [m.start() for m in re.finditer(r"bulk_commit\(\)", text)]
+  assert len(at) == 2
+  for a in at:      # in the branch of lane 0 alone, not in that of warps with rows
+    before = text[:a]
+    branch = before[before.rindex("if (lane == 0"):]
+    assert branch.startswith("if (lane == 0) {") and branch.count("{") - branch.count("}") == 1
+
+
 def test_the_kernel_has_no_other_report_of_a_landed_stage():
   """Arrivals of the odd CTA's threads on the even CTA's barriers: only of the epilogue, behind the tcgen05 fence."""
   text = re.sub(r"//[^\n]*", "", open(SOURCE).read())

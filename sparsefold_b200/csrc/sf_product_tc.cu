@@ -142,7 +142,9 @@ int product_tc(const Operand& a, const Operand& b, const Operand* b2, const Epi&
   // (1.1e-9 of a value per column), and a sum over the rows does not average that away (K = 2048, gated silu, dbias
   // against fp64: 2.2e-6 in segments of 2048, 5.1e-7 in these; 2000 rows of 4096 columns 33 us either way).
   // (dbias may be asked for without a bias: colpart; saved ones only serve it where the layer has one)
-  p.seg_kb = p.pairs > 1 || e.colpart || (e.bias && e.saved) ? 8 : p.nkb;
+  // Of 65536 for the rest, as a weight gradient's rows may be: a sum of one sign loses 3.8e-9 per column (dW over 3 million
+  // rows was short by 1.2 %), so 2.5e-4 at most here, a fourteenth of a bf16 result's rounding.
+  p.seg_kb = p.pairs > 1 || e.colpart || (e.bias && e.saved) ? 8 : p.nkb < 1024 ? p.nkb : 1024;
   // a plain sum's K may be split over CTAs
   const bool plain = e.kind == kLinear && e.act == SF_POST_NONE && !e.bias && !e.aux && !e.saved;
   const Plan plan = plan_of(p.m, p.n, p.nkb, p.pairs, p.seg_kb, gated, b.k_major, plain, sms);

@@ -64,8 +64,8 @@ struct Params {
 
 // Segments.  The tensor cores cut what does not fit their accumulator, always towards zero, so a sum loses about
 // 1.1e-9 of itself per unit of K (measured: 4.7e-7 at K = 512, 9e-6 at 8192).  Where the result has to be good to
-// fp32 (split fp32 operands; pre-activations whose gradient is summed over the rows for dbias), K is cut into
-// segments: each starts a new accumulator, and the epilogue warps add it, rounding to nearest, to a sum
+// fp32 (split fp32 operands; pre-activations whose gradient is summed over the rows for dbias), and where it is very long,
+// K is cut into segments: each starts a new accumulator, and the epilogue warps add it, rounding to nearest, to a sum
 // that waits in TMEM (columns kTotal on) until the last one.
 constexpr int kTotal = 256;
 // An accumulator's place and the parity of its use `it`.
@@ -568,7 +568,7 @@ __device__ __forceinline__ void add_bias(const float* bias, bool vec, int count,
   }
 }
 
-// LEAN: without bias, residual, saved pre-activations and column sums, decided when compiled: what a transition's
+// LEAN: without bias, residual, saved pre-activations, column sums and segments, decided when compiled: what a transition's
 // three products are, and worth 10 % of them at K = 128 (65536 x 128 -> 1024: 28 us against 32).
 // The epilogue warps' part of the kernel: bf16 out (activation EACT), or fp32 out (EACT < 0: p.act decides; exact
 // functions).
@@ -1189,7 +1189,7 @@ template <int KIND>
 int launch_staged_bf16(int ctas, const Maps& tm, const Params& p, cudaStream_t stream) {
   if constexpr (KIND != kDLinear) {
     constexpr int own = KIND == kLinear ? SF_POST_NONE : SF_POST_SILU;
-    if (p.act == own && !p.two && !p.bias && !p.saved && !p.colpart && (KIND != kLinear || !p.aux))
+    if (p.act == own && !p.two && p.kb_split <= p.seg_kb && !p.bias && !p.saved && !p.colpart && (KIND != kLinear || !p.aux))
       return launch_ctas<KIND, kOutBf16, true, own, true>(ctas, tm, p, stream);
   }
   int st = SF_OK;

@@ -177,6 +177,33 @@ def test_a_stack_trains_its_last_transitions_and_says_so():
         assert i == 0 or (bool(torch.isfinite(p.grad).all()) and bool(p.grad.any()))
 
 
+@pytest.mark.parametrize("rows,k,n,act,kn", [(40, 4_000_000, 64, "relu", False), (40, 4_000_003, 64, None, True),
+                                             (300, 2_600_000, 300, "relu", False)])
+def test_very_long_sums(rows, k, n, act, kn):
+  """Sums of millions of positive bf16 products.  The tensor cores' accumulator cuts some 1e-9 of the sum for each column,
+  over 0.004 for four million where the sum is not taken in pieces; rounding the result leaves 2^-9 of the norm at most."""
+  x = (rnd(1, rows, k).uniform_(0.5, 1.5)).to(BF)
+  w = (rnd(2, k, n).uniform_(0.5, 1.5) / k).to(BF).t() if kn else (rnd(2, n, k).uniform_(0.5, 1.5) / k).to(BF)
+  ref = sum(x[:, i:i + 200_000].double() @ w[:, i:i + 200_000].double().t() for i in range(0, k, 200_000))
+  assert gap(ops.linear_act(x, w, activation=act), ref) <= 2.0 ** -9
+  both = torch.cat((w, w))
+  one = ops.gated_linear(x, both, activation="relu")
+  assert gap(one, ref * ref) <= 2.0 ** -9
+
+
+def test_very_long_weight_gradients():
+  """The same over the rows: dW of enough tiles that the rows are not split over the CTAs."""
+  rows, k, n = 3_000_000, 1536, 1600
+  x, dy = torch.empty(rows, k, dtype=BF, device="cuda"), torch.empty(rows, n, dtype=BF, device="cuda")
+  ref = torch.zeros(n, k, dtype=torch.float64, device="cuda")
+  for i in range(0, rows, 100_000):
+    x[i:i + 100_000] = torch.rand(100_000, k, device="cuda") + 0.5
+    dy[i:i + 100_000] = torch.rand(100_000, n, device="cuda") + 0.5
+    ref += dy[i:i + 100_000].double().t() @ x[i:i + 100_000].double()
+  w = torch.zeros(n, k, dtype=BF, device="cuda")
+  assert gap(ops.linear_act_backward(dy, x, w, need_dx=False)[1], ref) <= 2.0 ** -9
+
+
 # ---- errors of whole tensors ------------------------------------------------------------------------------
 # Elementwise bounds over all magnitudes are far above what random signs leave, so that a term or a row may be missing
 # within them.  Norm of the error over norm of the result, instead, with e = 6.8e-7 for one fp32 product: a sum of 512

@@ -488,3 +488,20 @@ def test_dx_in_the_place_of_dy(rows, cols, sums, dtype):
   assert torch.equal(dy, want[0]) and bool((ws[need:] == 0x5A).all())
   if sums:
     assert torch.equal(dw, want[1]) and torch.equal(db, want[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,k,n", [(8, 200, 96), (20, 200, 96), (301, 1100, 130), (9400, 72, 600)])
+def test_a_row_does_not_depend_on_the_values_of_others(rows, k, n, dtype):
+  """y and dx of a row have the same bits whatever the other rows hold, large values among them."""
+  w, b, dy = (rnd(1, 2 * n, k) / k ** 0.5).to(dtype), rnd(2, 2 * n), rnd(3, rows, n).to(dtype)
+  x, other = rnd(4, rows, k).to(dtype), (1000 * rnd(5, rows, k)).to(dtype)
+  mine = torch.arange(rows, device="cuda") % 3 == 1
+  mixed, dy2 = torch.where(mine[:, None], x, other), torch.where(mine[:, None], dy, dy.flip(0))
+  for save in (False, True):
+    a, s = ops.gated_linear(x, w, b, save=True)
+    c, t = ops.gated_linear(mixed, w, b, save=True)
+    assert torch.equal(a[mine], c[mine])
+    u = ops.gated_linear_backward(dy, x, w, b, saved=s if save else None, need_dwt=False)[0]
+    v = ops.gated_linear_backward(dy2, mixed, w, b, saved=t if save else None, need_dwt=False)[0]
+    assert torch.equal(u[mine], v[mine])
